@@ -8,15 +8,15 @@ PARITY PINNING.  The reference has no tests, no golden outputs and no CPU path, 
 be built or run in the build container (Rust + gfx-hal + Vulkan are absent), so parity is
 UNPINNED BY THE REFERENCE'S OWN TESTS.  What pins this oracle instead:
   * the reference's two input files (tests/golden/{spectrum,omega}.bin, data);
-  * oracle/spirv_interp.py, which executes the reference's *shipped SPIR-V binaries*
-    (shader/spv/*.comp.spv, the code the reference actually runs) in the build container on those
-    inputs; its outputs are committed as tests/golden/spirv_frame512_t*.npz and the
-    ``*_literal`` functions below reproduce them BIT FOR BIT at every stage
-    (tests/test_oracle.py::test_literal_oracle_reproduces_the_shipped_spirv_bit_for_bit);
   * two independent formulations that must agree to ~1e-6
-    (``*_literal`` = fp32 restatement of the shaders instruction by instruction,
+    (``*_literal`` = fp32 restatement of the GLSL sources operation by operation,
     ``frame_f64`` = closed-form fp64 with numpy's pocketfft);
+  * the outputs of the ``*_literal`` functions on those inputs, committed as
+    tests/golden/literal_frame512_t*.npz and compared BIT FOR BIT at every stage, so that the
+    restatement cannot drift
+    (tests/test_oracle.py::test_literal_oracle_reproduces_its_committed_frames_bit_for_bit);
   * the survey-time KAT table (tests/golden/kat_survey.json).
+Parity with an execution of the reference itself is therefore unpinned.
 Driver-defined precision (sin, cos, length, division, FMA contraction) is fixed to "correctly
 rounded fp32, no contraction"; the reference's own GPU result is implementation-defined at that level.
 

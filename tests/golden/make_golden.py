@@ -8,10 +8,16 @@ Outputs (small, data only):
   frame512_t{0,1,10}.npz -- fp64-oracle output on data/*.bin: 64x64 top-left crop (as f32),
                          six probe texels and per-channel sum / l2 / max aggregates.
   frame256_t1.npz     -- same for the N=256 centre crop.
+  literal_frame512_t{0,1,10}.npz -- output of the literal fp32 restatement of the four GLSL shaders on
+                         data/*.bin: 64x64 crop and an every-8th-texel subsample of the RGBA32F image,
+                         per-channel aggregates, and CRC-32 of the raw bytes of the image and of every
+                         intermediate buffer after each dispatch group (propagate, fft_row x3, fft_col x3)
+                         in the order height, disp_x, disp_z.
 """
 import json
 import os
 import sys
+import zlib
 
 import numpy as np
 
@@ -49,12 +55,25 @@ def dump(name, out64):
         sum=ch.sum((0, 1)), l2=np.sqrt((ch ** 2).sum((0, 1))), max=np.abs(ch).max((0, 1)))
 
 
+def dump_literal(name, h0, om, t):
+    img, st = oc.frame_literal(h0, om, t, return_stages=True)
+    ch = img[..., :3].astype(np.float64)
+    crcs = {out: np.array([zlib.crc32(np.ascontiguousarray(b, np.complex64).tobytes()) for b in st[key]], np.uint32)
+            for key, out in (("propagate", "crc_propagate"), ("rows", "crc_fft_row"), ("cols", "crc_fft_col"))}
+    np.savez_compressed(
+        os.path.join(HERE, name),
+        crop=img[:64, :64].copy(), sub8=img[::8, ::8].copy(),
+        crc_image=np.uint32(zlib.crc32(img.tobytes())),
+        sum=ch.sum((0, 1)), l2=np.sqrt((ch ** 2).sum((0, 1))), max=np.abs(ch).max((0, 1)), **crcs)
+
+
 def main():
     with open(os.path.join(HERE, "kat_survey.json"), "w") as f:
         json.dump(KAT, f, indent=1)
     h0, om = oc.load_reference_inputs(os.path.join(HERE, "spectrum.bin"), os.path.join(HERE, "omega.bin"))
     for t in (0, 1, 10):
         dump(f"frame512_t{t}.npz", oc.frame_f64(h0, om, float(t)))
+        dump_literal(f"literal_frame512_t{t}.npz", h0, om, float(t))
     dump("frame256_t1.npz", oc.frame_f64(oc.centre_crop(h0, 256), oc.centre_crop(om, 256), 1.0))
 
 

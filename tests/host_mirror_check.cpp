@@ -6,8 +6,8 @@
 //       `Renderer::render` sit (src/render.rs:223-225, 742-924, 1101-1310): decode the reference's bincode
 //       inputs, upload, record the 8 staged dispatches (ocean_host::render) and the fused frame (Device::frame)
 //       at N = 512, and compare the top-left 64 x 64 texels of each displacement map with the golden crop
-//       (raw float32 [64][64][4], exported by the test from tests/golden/spirv_frame512_t1.npz = the
-//       reference's shipped SPIR-V executed on the same inputs).  Exit code 0 = both within 1e-4.
+//       (raw float32 [64][64][4], exported by the test from tests/golden/literal_frame512_t1.npz = the
+//       literal restatement of the reference's GLSL shaders on the same inputs).  Exit code 0 = both within 1e-4.
 #include <cmath>
 #include <cstdint>
 #include <cstdio>

@@ -1,8 +1,8 @@
 """GPU tier: NATIVE callers drive the C ABI.  A C++ program through the host mirror
 (csrc/host/ocean.hpp: Device / Propagation / Fft / Correction / render, what src/render.rs:223-225 and
 :1101-1310 would bind) and a plain C99 program through include/ocean_hip.h decode the reference's own bincode
-inputs, run the frame at N = 512, t = 1 on the GPU and compare with the golden crop produced by executing the
-reference's shipped SPIR-V (tests/golden/spirv_frame512_t1.npz).  No Python between the caller and the library."""
+inputs, run the frame at N = 512, t = 1 on the GPU and compare with the golden crop of the literal restatement of the
+reference's GLSL shaders (tests/golden/literal_frame512_t1.npz).  No Python between the caller and the library."""
 import os
 import subprocess
 
@@ -26,7 +26,7 @@ def _build(tmp_path, compiler, std, src, name):
 
 
 def _crop_file(tmp_path):
-    crop = np.load(os.path.join(GOLDEN, "spirv_frame512_t1.npz"))["crop"]      # float32 [64, 64, 4]
+    crop = np.load(os.path.join(GOLDEN, "literal_frame512_t1.npz"))["crop"]      # float32 [64, 64, 4]
     path = str(tmp_path / "crop.f32")
     np.ascontiguousarray(crop, dtype="<f4").tofile(path)
     return path

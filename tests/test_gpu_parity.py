@@ -144,10 +144,10 @@ def test_committed_golden_vectors(r512, r256, name, n, t):
 
 
 @pytest.mark.parametrize("t", [0, 1, 10])
-def test_against_the_reference_spirv_outputs(r512, t):
-    """HIP (fused and staged) vs vectors obtained by executing the reference's shipped
-    shader/spv/*.comp.spv on data/*.bin (tests/golden/make_spirv_golden.py)."""
-    gold = np.load(os.path.join(GOLDEN, f"spirv_frame512_t{t}.npz"))
+def test_against_the_literal_restatement_of_the_shaders(r512, t):
+    """HIP (fused and staged) vs the literal fp32 restatement of the reference's GLSL shaders on
+    data/*.bin (tests/golden/make_golden.py)."""
+    gold = np.load(os.path.join(GOLDEN, f"literal_frame512_t{t}.npz"))
     scale = gold["max"].max()
     for mode in ("fused", "staged"):
         (r512.render_fused if mode == "fused" else r512.render)(float(t))
