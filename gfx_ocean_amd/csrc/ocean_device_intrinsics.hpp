@@ -98,27 +98,25 @@ template <int T> __device__ __forceinline__ void line_sync() {
 }
 
 // Timeline probes for tools/timeline.hip (compiled in only with -DOCEAN_TIMELINE; the product build has none):
-// lane 0 of a workgroup records the 100 MHz wall clock at a few points, slot 15 the hardware id.
+// a workgroup records the 100 MHz wall clock at a few points, slot 15 the hardware id.
 #ifdef OCEAN_TIMELINE
 __device__ unsigned long long* ocean_tl;
-// scalar-only probe (no lane branch, no VGPRs: a lane-0 branch moved the register allocation of pass 1 from 9 to
-// 112 spills); every wave of the workgroup writes the slot, the last one wins
-__device__ __forceinline__ unsigned long long* ocean_tl_uniform(unsigned long long* p) {
-    const unsigned long long v = (unsigned long long)p;
-    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
-    return (unsigned long long*)(((unsigned long long)hi << 32) | lo);
+// Every lane of every wave of the workgroup stores the same slot, the last one wins: no lane branch (a lane-0 branch moved
+// the register allocation of pass 1 from 9 to 112 spills).  An agent-scope relaxed atomic store is one 8-byte vector
+// store past the L1 (defined although several waves write the slot); the ring of pass 1 counts it among its outstanding
+// memory instructions, so its waits come out no shorter.
+__device__ __forceinline__ void ocean_tl_store(unsigned long long* slot, unsigned long long v) {
+    __hip_atomic_store(slot, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ void ocean_tl_probe(unsigned long long* slot) {
     unsigned long long t;
-    slot = ocean_tl_uniform(slot);
-    asm volatile("s_memrealtime %0\n\ts_waitcnt lgkmcnt(0)\n\ts_store_dwordx2 %0, %1, 0x0\n\ts_dcache_wb" : "=&s"(t) : "s"(slot) : "memory");
+    asm volatile("s_memrealtime %0\n\ts_waitcnt lgkmcnt(0)" : "=s"(t) : : "memory");
+    ocean_tl_store(slot, t);
 }
 __device__ __forceinline__ void ocean_tl_hwid(unsigned long long* slot) {
     unsigned lo, hi;
-    slot = ocean_tl_uniform(slot);
     asm volatile("s_getreg_b32 %0, hwreg(HW_REG_HW_ID)\n\ts_getreg_b32 %1, hwreg(HW_REG_XCC_ID)" : "=s"(lo), "=s"(hi));
-    const unsigned long long id = ((unsigned long long)hi << 32) | lo;
-    asm volatile("s_store_dwordx2 %0, %1, 0x0\n\ts_dcache_wb" : : "s"(id), "s"(slot) : "memory");
+    ocean_tl_store(slot, ((unsigned long long)hi << 32) | lo);
 }
 #define OCEAN_TL(k)                                                            \
     do {                                                                       \

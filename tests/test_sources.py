@@ -29,3 +29,9 @@ def hits(pattern):
 def test_no_code_reads_the_references_compiled_shaders():
     """The oracle is written from the GLSL sources; nothing opens or decodes the modules compiled from them."""
     assert hits(re.compile(r"\.spv\b|/spv\b|\bspir-?v", re.I)) == []
+
+
+def test_no_code_writes_through_the_scalar_data_cache():
+    """Device code writes through vector stores only (scalar stores, scalar atomics and the cache's write-back and discard
+    are in no source, in inline assembly or comments): the timeline probes wrote their slots with scalar stores."""
+    assert hits(re.compile(r"(\b|\\[nt])s_((buffer_|scratch_)?(store|atomic)|dcache_(wb|discard))")) == []
