@@ -27,15 +27,15 @@
 
 namespace ocean {
 
-// c32 (ocean_device_intrinsics.hpp) is a packed (re, im) 2-vector; everything here is written in whole-vector
-// operations so that each line below is ONE v_pk_* instruction (swizzles ride on op_sel, constants in SGPR pairs).
+// c32 (ocean_device_intrinsics.hpp) is a (re, im) 2-vector; everything here is written in whole-vector operations, each of
+// them one instruction per lane (swizzles and the signs of +-1 constants cost nothing).
 __device__ __forceinline__ c32 cadd(c32 a, c32 b) { return a + b; }
 __device__ __forceinline__ c32 csub(c32 a, c32 b) { return a - b; }
 __device__ __forceinline__ c32 cadd_i(c32 a, c32 b) { return vfma(yx(b), mk(-1.0f, 1.0f), a); }   // a + i b
 __device__ __forceinline__ c32 csub_i(c32 a, c32 b) { return vfma(yx(b), mk(1.0f, -1.0f), a); }   // a - i b
 __device__ __forceinline__ c32 crot(c32 a) { return yx(a) * mk(-1.0f, 1.0f); }                    // i a
 __device__ __forceinline__ c32 cconj(c32 a) { return a * mk(1.0f, -1.0f); }
-// a * w given w and wr = i w: two instructions; without wr: three, no temporary twiddle
+// a * w given w and wr = i w: two operations; without wr: three, no temporary twiddle
 __device__ __forceinline__ c32 cmul_r(c32 a, c32 w, c32 wr) { return vfma(yy(a), wr, xx(a) * w); }
 __device__ __forceinline__ c32 cmul(c32 a, c32 w) { return vfma(yy(a) * yx(w), mk(-1.0f, 1.0f), xx(a) * w); }
 
@@ -146,7 +146,7 @@ template <int N> struct LdsLine { static constexpr int elems = N + (N >> 4); };
 // a[t] *= w^t, t in [0, R).  For R > 4 the rotation is split in two levels, t = 4*t1 + t2:
 // w^t = (w^4)^t1 * w^t2, so only {w, w^2, w^3} and the powers of w^4 are ever live instead of an (R-1)-entry power
 // table.  The three low powers are kept together with their rotated copies i w^t2 (each is used by R/4
-// products, which then cost two packed instructions); the high powers use the three-instruction product.
+// products, which then cost two two-lane operations); the high powers use the three-operation product.
 // R <= 16: the high powers w^4, w^8, w^12 are products (depth <= 5, a few ulp on the twiddle).
 // R >= 32: they are read from the twiddle table (tw[(4 t1 step) mod table]: exact entries, L1-resident) -- a
 // product chain would be 7 or 15 deep.

@@ -34,11 +34,10 @@ __device__ __forceinline__ void jittered_syncthreads() {
 #define __syncthreads() ::ocean::jittered_syncthreads()
 #endif
 
-// A complex number is a 2-vector of floats living in an even-aligned VGPR pair, so that complex arithmetic
-// maps onto gfx950's packed fp32 instructions (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32: two lanes per
-// instruction, swizzles through op_sel): pass 1's phases are VALU-issue-bound (tools/timeline.hip), and the
-// packed form halves the instruction count of the butterflies.  The vector primitives below are the whole
-// interface; tests/hipemu has scalar twins.
+// A complex number is a 2-vector of floats, and complex arithmetic is written in whole-vector operations.  The library is
+// compiled without gfx950's packed fp32 arithmetic (hipcc_command in _lib.py says why and what it costs), so each of them is
+// two fp32 instructions: a swizzle then is a choice of register and a +-1 factor a sign on an operand, at no cost.
+// The vector primitives below are the whole interface; tests/hipemu has scalar twins.
 typedef float c32 __attribute__((ext_vector_type(2)));
 __host__ __device__ __forceinline__ c32 mk(float re, float im) { return c32{re, im}; }
 __host__ __device__ __forceinline__ c32 xx(c32 a) { return __builtin_shufflevector(a, a, 0, 0); }

@@ -68,7 +68,7 @@ __device__ __forceinline__ c32 propagate_height(c32 h0, c32 h0_neg, float omega,
     const float turns = rintf(disp * INV_2PI_HI);
     const float frac = fmaf(disp, INV_2PI_LO, fmaf(disp, INV_2PI_HI, -turns));
     const float s = sin_rev(frac), c = cos_rev(frac);
-    // h0 (c + i s) + h0_neg (c - i s) = c (h0 + h0_neg) + s * i (h0 - h0_neg): five packed instructions
+    // h0 (c + i s) + h0_neg (c - i s) = c (h0 + h0_neg) + s * i (h0 - h0_neg): five two-lane operations
     const c32 p = h0 + h0_neg, q = h0 - h0_neg;
     return vfma(yx(q) * s, mk(-1.0f, 1.0f), p * c);
 }
@@ -170,7 +170,7 @@ constexpr int CHUNK_W = 4, CHUNK_R = 4;
 // One field's symmetrised column spectrum (times 2) at row y of a column pair; kxv = (k(x), k((N-x)%N)).
 // 2 S(H) = A + B,  2 S(Dx) = i (k2.x B - k1.x A),  2 S(Dz) = i (k2.y B - k1.y A),  k1 = k_norm(x, y),
 // k2 = k_norm((N-x)%N, (N-y)%N) with the Q1 wrap and k * rsqrt(|k|^2) (k_normalised_fast), evaluated for
-// the pair (k1, k2) in the two lanes of packed instructions.
+// the pair (k1, k2) in the two lanes of one vector.
 template <int N>
 __device__ __forceinline__ c32 half_spectrum_at(int f, c32 A, c32 B, c32 kxv, float kscale, int y) {
     if (f == 1) return A + B;
@@ -197,7 +197,7 @@ __device__ __forceinline__ void half_spectrum(int f, const c32 (&A)[E], const c3
 // one after the other): height first (2 S(H) = A + B from the unscaled values), then A <- A / |k1|, B <- B / |k2| in place
 // (half_scale_AB: the one place the two quarter-rate v_rsq_f32 per element are paid), after which
 //     2 S(Dx) = i (k2.x B' - k1.x A'),   2 S(Dz) = i (k2.y B' - k1.y A')
-// are three packed instructions per element (k.x is the column's, wave-uniform; k.y a conversion and a multiply).  The
+// are three two-lane operations per element (k.x is the column's, wave-uniform; k.y a conversion and a multiply).  The
 // transform phases of pass 1 are VALU-issue-bound and the two normalisations were 2 x 2.3 of their 22 us per round at
 // N = 4096: frame 0.186 -> 0.181-0.182 ms, 5366-5374 -> 5488-5538 frames/s (r04_run18, A/B on one box); and the kernel drops
 // from 128 VGPRs with 6 spilled to 124 with none.  (A / |k| * k.x instead of A * (k.x / |k|): one rounding moved, 1 ulp.)
@@ -590,7 +590,7 @@ k_half_pass1(const void* __restrict__ h0T, float descale, const float* __restric
 #pragma unroll
     for (int ff = 0; ff < (FPAR ? 1 : 3); ++ff) {
         // One field group per field (FPAR), or the three fields one after the other: height first, then A and B are
-        // normalised in place and disp_x, disp_z cost three packed instructions per element (half_scale_AB).
+        // normalised in place and disp_x, disp_z cost three two-lane operations per element (half_scale_AB).
         constexpr bool SHARED_R = SHR;
         static_assert(!(FPAR && SHR), "one field per wave group: nothing to share");
         const int f = FPAR ? fg : ((ff == 0) ? 1 : ((ff == 1) ? 0 : 2));

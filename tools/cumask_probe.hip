@@ -1,7 +1,7 @@
 // cumask_probe.hip -- which CUs does a stream created with hipExtStreamCreateWithCUMask run on?  (For an experiment that runs pass 1
 // of frame f + 1 and pass 2 of frame f side by side on disjoint sets of CUs.)  Launches many one-wave workgroups that record
 // XCC_ID and HW_ID on a masked stream and prints, per mask, how many distinct CUs of every XCD were seen.
-//   hipcc --offload-arch=gfx950 -O3 -o cumask_probe cumask_probe.hip
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o cumask_probe cumask_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

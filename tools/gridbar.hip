@@ -3,7 +3,7 @@
 // 256 co-resident workgroups (one per CU, 256 threads) meet at K device-scope barriers: each workgroup writes 12 KiB of an
 // "intermediate" with write-through stores, arrives on an atomic counter in fine-grained (system-scope) fashion, spins
 // until all have arrived, then reads 12 KiB that OTHER workgroups (other XCDs) wrote, bypassing its XCD's L2.
-//   hipcc --offload-arch=gfx950 -O3 tools/gridbar.hip -o tools/gridbar && tools/gridbar
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/gridbar.hip -o tools/gridbar && tools/gridbar
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,7 +1,7 @@
 // membench.hip -- calibration microbenchmarks for the roofline numbers in DESIGN.md:
 // plain float4 copy (the chip's achievable HBM rate) and the two access patterns the fused
 // kernels add on top of it (chunked gather with a large power-of-two-ish stride).
-// Build: hipcc --offload-arch=gfx950 -O3 tools/membench.hip -o tools/membench ; run on the GPU box.
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/membench.hip -o tools/membench ; run on the GPU box.
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

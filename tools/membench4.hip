@@ -2,7 +2,7 @@
 // (1) read bandwidth of a buffer re-read every launch, by footprint; (2) the same 192 MiB buffer re-read with a
 // 512 MiB streaming write (plain / non-temporal stores) between the reads -- the shape of a frame loop whose
 // static inputs (201 MB at N = 4096) would like to stay cached while 670 MB of intermediates stream by.
-// Build: hipcc --offload-arch=gfx950 -O3 tools/membench4.hip -o tools/membench4
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/membench4.hip -o tools/membench4
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

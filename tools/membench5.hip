@@ -4,7 +4,7 @@
 // the others compute, a chip-level stagger of the load phases would shorten them.  This measures exactly that: G workgroups of
 // 1024 threads (one per CU, 160 KiB of LDS requested so that no two share a CU) each stream SPAN bytes from their own region,
 // through VGPRs (dwordx4, UNROLL loads in flight per lane) or through LDS-DMA (global_load_lds_dwordx4, a ring), REPS regions
-// per workgroup so that nothing is cache-resident.       hipcc --offload-arch=gfx950 -O3 -o membench5 membench5.hip
+// per workgroup so that nothing is cache-resident.       hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o membench5 membench5.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
