@@ -88,8 +88,7 @@ class CorrectionLocalsC(ctypes.Structure):
 # gfx950 code without packed fp32 arithmetic: some forms of those instructions have given wrong values now and then on
 # MI355X, with no error and not reproducibly.  hipcc makes them of every two-lane float operation unless the feature is
 # off (its host pass warns that it does not know the feature: harmless).  One box, both builds in turn, us a frame with /
-# without them: 256 8.0 / 8.8, 512 9.7 / 9.9, 1024 20.3 / 21.5, 2048 44.5 / 44.4, 4096 175 / 179, 8192 766 / 776 (fp16
-# spectrum with the 16-bit intermediate: 778 / 820, its pass 2 then spills 11 VGPRs).
+# without them: 256 8.0 / 8.8, 512 9.7 / 9.9, 1024 20.3 / 21.5, 2048 44.5 / 44.4, 4096 175 / 179, 8192 766 / 776.
 NO_PACKED_FP32 = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
 
 

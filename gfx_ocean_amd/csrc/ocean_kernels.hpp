@@ -1034,7 +1034,7 @@ k_half_pass2_real(const c32* __restrict__ inter, float4* __restrict__ out, const
     const uint32_t sx = (uint32_t)lay.sx, fs = (uint32_t)lay.fs;
     const uint32_t offy = (uint32_t)chunk_row_offset(lay, y / CR) + (uint32_t)((tid % P1) * CR + (y % CR));   // column-major chunks (k_half_pass1_split)
     constexpr uint32_t SF = (uint32_t)(N / 64) * (N / 4);          // I16: one field's scales
-    // the E half-spectrum values kx = tid + e T of field f (I16: the raw int16 pair in .x, its scale in .y)
+    // the E half-spectrum values kx = tid + e T of field f (I16: the raw int16 pair in .x, its scale, issue_scales, in .y)
     auto issue = [&](int f, c32 (&raw)[E]) {
         const char* base = reinterpret_cast<const char*>(inter);
 #pragma unroll
@@ -1047,20 +1047,31 @@ k_half_pass2_real(const c32* __restrict__ inter, float4* __restrict__ out, const
                 raw[e] = *reinterpret_cast<const c32*>(base + (size_t)(o * 8u));
             } else if constexpr (I16) {
                 const uint32_t o = (uint32_t)f * fs + offy + Xc * sx;
-                const float* sc = inter_scale + ((uint32_t)f * SF + (uint32_t)(y >> 6) * (N / 4) + (uint32_t)(tid >> 1) + e * (T / 2));
-                raw[e] = mk(*reinterpret_cast<const float*>(base + (size_t)(o * 4u)), sc[0]);
+                raw[e].x = *reinterpret_cast<const float*>(base + (size_t)(o * 4u));
             } else {
                 const uint32_t o = (uint32_t)f * fs + offy + Xc * sx;
                 raw[e] = *reinterpret_cast<const c32*>(base + (size_t)(o * 8u));
             }
         }
     };
+    // I16: the scales of field f.  Those of disp_x and disp_z are loaded behind the transform before them, not with the values:
+    // 16 VGPRs fewer per field in flight (119 and no spill; 128 and 11 spilled with both together), and at N = 8192 this
+    // kernel takes 339 instead of 465 us, the same bits.
+    auto issue_scales = [&](int f, c32 (&raw)[E]) {
+        if constexpr (I16) {
+            const float* sc = inter_scale + ((uint32_t)f * SF + (uint32_t)(y >> 6) * (N / 4));   // wave-uniform
+            const uint32_t o = (uint32_t)(opaque_lane(tid) >> 1);
+#pragma unroll
+            for (int e = 0; e < E; ++e) raw[e].y = (sc + e * (T / 2))[o];
+        }
+    };
     float keep_h[2 * E], keep_x[2 * E];
     const c32 wj = tw[tid];                                        // e^{2 pi i j / N}: once, for the three fields
     const float sgn = (((tid + y) & 1) == 0) ? -0.5f : 0.5f;       // correction.comp:29 and the 1/2 of S(F); T is even
     float4* orow = out + (size_t)y * N;
-    // one field: pair, transform, take the store mapping.  `after_pairing` issues the loads that replace raw's registers.
-    auto field = [&](int it, const c32 (&raw)[E], auto&& after_pairing) {
+    // one field: pair, transform, take the store mapping.  `after_pairing` issues the loads that replace raw's registers,
+    // `after_transform` the next field's scales.
+    auto field = [&](int it, const c32 (&raw)[E], auto&& after_pairing, auto&& after_transform) {
         const int jf = opaque_lane(tid);
         if (it > 0) __syncthreads();                               // the previous field's store-mapped reads are done
         c32* lo = line + lds_pad(jf);
@@ -1077,6 +1088,7 @@ k_half_pass2_real(const c32* __restrict__ inter, float4* __restrict__ out, const
         if (it == 0) OCEAN_TL(1);
         fft_line_to_lds<M, E, 2, true, FUSED_HWTW>(reg, jf, tw, line);
         if (it == 2) OCEAN_TL(5);
+        after_transform();
         const float* src = reinterpret_cast<const float*>(line + lds_pad(jf >> 1)) + (jf & 1);
         if (it == 0) {
 #pragma unroll
@@ -1096,12 +1108,13 @@ k_half_pass2_real(const c32* __restrict__ inter, float4* __restrict__ out, const
     OCEAN_TL(0);
     c32 raw_h[E], raw_x[E], raw_z[E];
     issue(1, raw_h);
+    issue_scales(1, raw_h);
     issue(0, raw_x);
-    field(0, raw_h, [&] { issue(2, raw_z); });
+    field(0, raw_h, [&] { issue(2, raw_z); }, [&] { issue_scales(0, raw_x); });
     OCEAN_TL(2);
-    field(1, raw_x, [] {});
+    field(1, raw_x, [] {}, [&] { issue_scales(2, raw_z); });
     OCEAN_TL(4);
-    field(2, raw_z, [] {});
+    field(2, raw_z, [] {}, [] {});
     OCEAN_TL(6);
 }
 
