@@ -10,7 +10,7 @@ namespace ocean {
 // untouched, so a frame of this build must be BIT-identical to the product build's; a missing or misplaced barrier --
 // two waves touching the same LDS words with only "they usually arrive in this order" between them -- shows up as a
 // difference within a few hundred frames (tests/test_gpu_race.py::test_barrier_jitter_build_is_bit_identical).
-// AddressSanitizer for the device is not available on this pool (xnack-, no instrumented runtime:
+// There is no AddressSanitizer run of the device code (xnack-, no instrumented runtime:
 // profiles/r03_run16_asan_attempt_log.txt).
 #ifdef OCEAN_RACE_JITTER   // (a test build: tests/test_gpu_race.py compiles it next to the product and compares checksums)
 __device__ __forceinline__ void race_jitter() {
